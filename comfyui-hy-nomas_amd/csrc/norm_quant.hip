@@ -305,13 +305,26 @@ __global__ __launch_bounds__(kThreads) void rms_norm_quant_kernel(const NormArgs
       if (k < CPL && has) sr[at / 16] = g.scale;
       return;
     }
-#pragma unroll 1
-    for (int c = first, i = 0; c < chunks; c += kStep, i++) {
-      float y[8];
-      const float sc = plain_scale<KIND>(row16_max(formula(i, y)));
-      st_nt8(qr + c * 8, plain_codes<KIND>(y, sc, a.rounding));
-      if (k == 0) sr[c / 16] = sc;
+    // Some group of the wave has no factor (pruned channels, say): it alone takes the formula, so that a group's codes never
+    // depend on what lies in another.
+    const float usable = g.ok ? 1.0f : 0.0f;
+#pragma unroll
+    for (int i = 0; i < CPL; i++) {
+      const float f = row_bcast(g.rcp, i);
+      const bool fast = row_bcast(usable, i) != 0.0f;  // the same in the group's 16 lanes
+      const int c = first + kStep * i;
+      if (c < chunks) {
+        if (fast) {
+          st_nt8(qr + c * 8, fast_codes<KIND>(t[i], f, __uint_as_float(peak[i]), a.rounding));
+        } else {
+          float y[8];
+          const float sc = plain_scale<KIND>(row16_max(formula(i, y)));
+          st_nt8(qr + c * 8, plain_codes<KIND>(y, sc, a.rounding));
+          if (k == 0) sr[c / 16] = sc;
+        }
+      }
     }
+    if (k < CPL && has && g.ok) sr[at / 16] = g.scale;
   }
 }
 
