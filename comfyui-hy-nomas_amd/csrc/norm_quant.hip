@@ -143,22 +143,41 @@ __device__ __forceinline__ uint2 plain_codes(const float* y, float scale, int ro
 }
 
 // t top / peak with the quotient's rounding error mended: where it lies halfway between two codes, as 1 in 2300 does with
-// 16-bit values and weights, it is formed exactly and goes to the code that the rounding says.  (A product with top / peak alone
-// gave half of those to the other neighbour.)
-template <int KIND>
+// bf16 values and weights, it is formed exactly and goes to the code that the rounding says.  (A product with top / peak alone
+// gave half of those to the other neighbour.)  A bf16 product h w has 16 bits, so t top is exact, and quotients that are no
+// ties lie further from one than fp32's rounding reaches.
+//
+// WIDE, fp16 values: t has up to 22 bits and t top up to 29, so its low part goes into the remainder, and a quotient may lie
+// within fp32's rounding of a tie.  The last remainder e tells on which side; z is made the odd neighbour of the quotient (the
+// quotient itself where e is 0), which no boundary of codes is, so that the rounding to a code sees what a quotient of
+// unlimited precision would show it.  The half-away sum takes the float below 0.5, whose sum with a value under a half stays under.
+template <int KIND, bool WIDE>
 __device__ __forceinline__ uint2 fast_codes(const float* t, float rcp, float peak, int rounding) {
+  constexpr float top = KIND == HN_KIND_FP8 ? 448.0f : 127.0f;
   float z[8];
 #pragma unroll
   for (int j = 0; j < 8; j++) {
-    const float n = t[j] * (KIND == HN_KIND_FP8 ? 448.0f : 127.0f), q = n * rcp;
-    z[j] = __builtin_fmaf(__builtin_fmaf(-q, peak, n), rcp, q);
+    const float n = t[j] * top, q = n * rcp;
+    if constexpr (WIDE) {
+      const float lo = __builtin_fmaf(t[j], top, -n);
+      const float near = __builtin_fmaf(__builtin_fmaf(-q, peak, n) + lo, rcp, q);
+      const float e = __builtin_fmaf(-near, peak, n) + lo;
+      const uint32_t bits = __float_as_uint(near);
+      const uint32_t below = (uint32_t)((int)(bits ^ __float_as_uint(e)) >> 31);  // -1 where the quotient is nearer to zero
+      z[j] = __uint_as_float(e == 0.0f ? bits : (bits + below) | 1u);
+    } else {
+      z[j] = __builtin_fmaf(__builtin_fmaf(-q, peak, n), rcp, q);
+    }
   }
   if constexpr (KIND == HN_KIND_FP8) {
     return make_uint2(e4m3_pack4_hw(z[0], z[1], z[2], z[3]), e4m3_pack4_hw(z[4], z[5], z[6], z[7]));
   } else {
     int c[8];
 #pragma unroll
-    for (int j = 0; j < 8; j++) c[j] = rounding == HN_ROUND_HALF_EVEN ? rne_code_bits(z[j]) : round_half_away_i8_inrange(z[j]);
+    for (int j = 0; j < 8; j++)
+      c[j] = rounding == HN_ROUND_HALF_EVEN ? rne_code_bits(z[j])
+             : WIDE                         ? (int)(z[j] + __builtin_copysignf(0x1.fffffep-2f, z[j]))
+                                            : round_half_away_i8_inrange(z[j]);
     return make_uint2(pack4_i8(c[0], c[1], c[2], c[3]), pack4_i8(c[4], c[5], c[6], c[7]));
   }
 }
@@ -254,7 +273,7 @@ __global__ __launch_bounds__(kThreads) void rms_norm_quant_kernel(const NormArgs
     if (__builtin_expect(g.ok, 1)) {  // the same in the whole row
 #pragma unroll
       for (int i = 0; i < CPL; i++)
-        if (first + kStep * i < chunks) st_nt8(qr + (first + kStep * i) * 8, fast_codes<KIND>(t[i], g.rcp, __uint_as_float(top), a.rounding));
+        if (first + kStep * i < chunks) st_nt8(qr + (first + kStep * i) * 8, fast_codes<KIND, DT == HN_DTYPE_F16>(t[i], g.rcp, __uint_as_float(top), a.rounding));
       if (first == 0) sr[0] = g.scale;
       return;
     }
@@ -300,7 +319,7 @@ __global__ __launch_bounds__(kThreads) void rms_norm_quant_kernel(const NormArgs
 #pragma unroll
       for (int i = 0; i < CPL; i++) {
         const float f = row_bcast(g.rcp, i);
-        if (first + kStep * i < chunks) st_nt8(qr + (first + kStep * i) * 8, fast_codes<KIND>(t[i], f, __uint_as_float(peak[i]), a.rounding));
+        if (first + kStep * i < chunks) st_nt8(qr + (first + kStep * i) * 8, fast_codes<KIND, DT == HN_DTYPE_F16>(t[i], f, __uint_as_float(peak[i]), a.rounding));
       }
       if (k < CPL && has) sr[at / 16] = g.scale;
       return;
@@ -315,7 +334,7 @@ __global__ __launch_bounds__(kThreads) void rms_norm_quant_kernel(const NormArgs
       const int c = first + kStep * i;
       if (c < chunks) {
         if (fast) {
-          st_nt8(qr + c * 8, fast_codes<KIND>(t[i], f, __uint_as_float(peak[i]), a.rounding));
+          st_nt8(qr + c * 8, fast_codes<KIND, DT == HN_DTYPE_F16>(t[i], f, __uint_as_float(peak[i]), a.rounding));
         } else {
           float y[8];
           const float sc = plain_scale<KIND>(row16_max(formula(i, y)));
