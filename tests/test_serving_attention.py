@@ -647,3 +647,35 @@ def test_entry_point_refusals_without_a_gpu():
         assert f(*([1, 4, 3, 1, 10, 10, 128] if n == 7 else [1, 4, 3, 1, 10, 128]), *more) == -1
         assert f(*([1, 4, 2, -1, 10, 10, 128] if n == 7 else [1, 4, 2, -1, 10, 128]), *more) == -1
         assert f(*([1, 4, 2, 1, 10, 10, 96] if n == 7 else [1, 4, 2, 1, 10, 96]), *more) == -1
+
+
+def far_rows(dev, dtype, g, step, n, d, at=0):
+    """[n, 1, d] values `step` elements apart in a store of their own."""
+    t = torch.as_strided(torch.empty(n * step + at + d, device=dev, dtype=dtype), (n, 1, d), (step, d, 1), at)
+    return t.copy_(heads(g, torch.float32, n, 1, d).to(dtype) if dtype.is_floating_point else
+                   torch.randint(-127, 128, (n, 1, d), generator=g).to(dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lq", [1, 40, 140])
+@pytest.mark.parametrize("int8", [False, True])
+def test_key_offsets_past_2_to_the_32(dev, lq, int8):
+    """600 keys of one sample at the largest token stride, 2^23 elements: a tile's offset from the sample's start passes 2^32
+    elements, 16-bit and int8 alike, and the scales' too, for few, half and whole blocks of rows."""
+    from hy_nomas import attention
+
+    g, step, n, d = seeded(lq), 1 << 23, 600, 128
+    bf = torch.bfloat16
+    q = heads(g, bf, 1, lq, 1, d).to(dev)
+    if int8:
+        prefix = tuple((far_rows(dev, torch.int8, g, step, n, d, 16 * i), far_rows(dev, torch.float32, g, step, n, 1).abs_().mul_(0.02))
+                       for i in range(2))
+        plain = tuple(tuple(t.contiguous() for t in p) for p in prefix)
+    else:
+        prefix = tuple(far_rows(dev, bf, g, step, n, d, 8 * i) for i in range(2))
+        plain = tuple(t.contiguous() for t in prefix)
+        got = attention.cross_attention(q, *(t[None] for t in prefix))
+        check_cross(got, q, *(t[None] for t in plain), seen_of(1, n, None, None))
+    k, v = (heads(g, bf, 1, 70, 1, d).to(dev) for _ in range(2))
+    got = attention.prefix_attention(q, prefix, k, v)
+    check_prefix(got, q, plain, k, v, None, False)
