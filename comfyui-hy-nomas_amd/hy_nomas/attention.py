@@ -318,6 +318,8 @@ def _serving_operands(who, q, k, v, lengths, out):
         o = (out, out.data_ptr(), lq * hq * d, d, hq * d)
     else:
         st = out.stride()
+        if out.shape == qs and (st[0] | st[1] | st[2]) & 3:  # (a dim of one element has no second row: its stride does not count)
+            st = *(0 if n == 1 else s for s, n in zip(st[:3], qs)), st[3]
         if (out.shape != qs or out.dtype is not dt or st[3] != 1 or out.data_ptr() & 7 or (st[0] | st[1] | st[2]) & 3):
             raise RuntimeError(f"{who}: out must be {dt} {tuple(qs)} with a contiguous head dim and 8-byte aligned rows")
         if out.device != dev:

@@ -679,3 +679,17 @@ def test_key_offsets_past_2_to_the_32(dev, lq, int8):
     k, v = (heads(g, bf, 1, 70, 1, d).to(dev) for _ in range(2))
     got = attention.prefix_attention(q, prefix, k, v)
     check_prefix(got, q, plain, k, v, None, False)
+
+
+@pytest.mark.gpu
+def test_an_output_whose_single_dims_have_odd_strides(dev):
+    """A dimension of one element has no second row to misalign: its stride does not count."""
+    from hy_nomas import attention
+
+    g, bf = seeded(5), torch.bfloat16
+    q, k, v = (heads(g, bf, 1, n, 2, 64).to(dev) for n in (3, 40, 40))
+    out = torch.as_strided(torch.zeros(2 * 386, device=dev, dtype=bf), (1, 3, 2, 64), (386, 128, 64, 1))
+    want = attention.cross_attention(q, k, v)
+    assert attention.cross_attention(q, k, v, out=out) is out and torch.equal(out, want)
+    out = torch.as_strided(torch.zeros(500, device=dev, dtype=bf), (1, 1, 2, 64), (7, 5, 64, 1))
+    assert torch.equal(attention.cross_attention(q[:, :1], k, v, out=out), attention.cross_attention(q[:, :1], k, v))
