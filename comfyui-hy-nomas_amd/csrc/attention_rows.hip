@@ -35,7 +35,9 @@
 // probability times a scale could leave, the reference is that of the products: scores plus the scales' logarithms.)
 //
 // Hidden keys.  A tile's seen keys are one 64-bit mask.  Rows that are not seen are loaded from a seen row of the tile, so that
-// nothing they hold enters a product; a tile without a seen key is passed over.
+// nothing they hold enters a product; a tile without a seen key is passed over.  Under a causal limit some rows of a tile see a
+// key that others do not, and a value of it that is not finite reaches these as 0 times it: a row with a result that is not
+// finite, and with keys that it does not see, is walked again by a wave over the keys that it sees (`mend_row`).
 //
 // Splits.  Where the rows leave compute units idle, several workgroups take ranges of the tiles and leave fp32 partials with
 // their reference maximum and sum, which row_combine_kernel joins; a prefix and the samples' own keys are joined the same way.
@@ -166,7 +168,7 @@ __device__ __forceinline__ float row_max_xor32(float x) {  // max over lanes l a
   return __builtin_fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
 }
 
-// this wave's loads are done, direct ones among them
+// this wave's loads are done, direct ones among them, and its stores, which the same counter holds
 __device__ __forceinline__ void wait_loads() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));  // vmcnt(0)
@@ -481,6 +483,15 @@ struct RowCore {
       }
   }
 
+  __device__ __forceinline__ bool finite() const {  // the lane's results
+    float x = 0.0f;
+#pragma unroll
+    for (int db = 0; db < DB; db++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) x = __builtin_fmaf(oacc[db][r], 0.0f, x);
+    return x == 0.0f;
+  }
+
   __device__ __forceinline__ float total() const { return lsum + __shfl_xor(lsum, 32); }
 };
 
@@ -493,6 +504,157 @@ __device__ __forceinline__ void store_codes(char* row, int swz, int c, v4i_r w) 
   *reinterpret_cast<uint4*>(row + (((2 * c + 1) ^ swz) << 4)) = make_uint4(b0.x, b0.y, b1.x, b1.y);
 }
 
+// One row's attention again, by a whole wave over the keys that the row sees and no others, in fp32: 64 keys a step, D / 8 lanes a
+// key and 8 dims a lane, for K and V alike.  For rows whose result is not finite under a causal limit although their scores are,
+// so that what a later token's values hold stays with the rows that see it; slow beside the tiles, and rare: 4 x 2000 queries over 8192
+and 2000 keys take 1.1 ms, with a NaN in one sample's last value 11, in the first own value of every sample (where the rows are
+walked again for nothing) 55.  A: keys of a lane whose
+// rows are loaded together (in a kernel of many registers all of a step's).  CODES: a source may hold int8 codes.
+template <int DT, int D, int A, bool CODES>
+__device__ __forceinline__ void mend_row(int src0, int nsrc, int b, int qi, int h, int lane) {
+  const RowArgs& a = *(const RowArgs*)__builtin_amdgcn_kernarg_segment_ptr();  // (as a reference handed on, the arguments are copied)
+  constexpr int L = D / 8, N = L;  // lanes of a key, keys of a lane in a step
+  constexpr int kAhead = A < N ? A : N;
+  const int chunk = lane % L, sub = lane / L, hk = a.by_g(h);
+  float q[8], o[8] = {}, m = -__builtin_inff(), l = 0.0f;
+  In<DT>::widen8(*reinterpret_cast<const uint4*>(a.q + b * a.sqb + h * a.sqh + qi * a.sqi + 8 * chunk), q);
+#pragma unroll
+  for (int i = 0; i < 8; i++) q[i] *= a.scale_log2;
+  auto walk = [&](const KeySource& s, auto coded_c) __attribute__((always_inline)) {
+    constexpr bool coded = decltype(coded_c)::value;
+    int n = (int)sample_length(s, b);
+    if (s.causal) n = max(0, min(n, n - (int)a.Lq + qi + 1));
+    constexpr int eb = coded ? 1 : 2;
+    const char* const k0 = (const char*)s.k + (b * s.skb + hk * s.skh) * eb;
+    const char* const v0 = (const char*)s.v + (b * s.svb + hk * s.svh) * eb;
+    const uint32_t kj = (uint32_t)s.skj * eb, vj = (uint32_t)s.svj * eb;
+    auto fetch = [&](__amdgpu_buffer_rsrc_t r, uint32_t at) {  // 8 values, or 8 codes in the first half
+      if constexpr (coded) {
+        const auto c = __builtin_amdgcn_raw_buffer_load_b64(r, at + 8 * chunk, 0, 0);
+        return v4i_r{(int)c[0], (int)c[1], 0, 0};
+      }
+      return load16(r, at + 16 * chunk, 0);
+    };
+    auto widen = [&](v4i_r w, float (&f)[8]) {
+      if constexpr (coded) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) f[i] = (float)(int)(int8_t)((uint32_t)w[i / 4] >> (8 * (i & 3)));
+      } else {
+        In<DT>::widen8(__builtin_bit_cast(uint4, w), f);
+      }
+    };
+    for (int key0 = 0; key0 < n; key0 += 64) {
+      const int here = n - key0;  // the lane's keys: key0 + sub + 64 / L * i, the last one of the row for those past it
+      const __amdgpu_buffer_rsrc_t kr = buffer_rsrc(k0 + (int64_t)key0 * kj), vr = buffer_rsrc(v0 + (int64_t)key0 * vj);
+      float sc[N], top = m;
+#pragma unroll
+      for (int i0 = 0; i0 < N; i0 += kAhead) {
+        int my = sub;
+        if constexpr (kAhead < N) asm volatile("" : "+v"(my)::"memory");  // (no more loads and places ahead than there are registers)
+        v4i_r w[kAhead];
+        float scale[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+          const int key = min(my + 64 / L * (i0 + u), here - 1);
+          w[u] = fetch(kr, key * kj);
+          scale[u] = coded ? s.ks[hk * s.ksh + (key0 + key) * s.ksj] : 1.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+          float f[8], x = 0.0f;
+          widen(w[u], f);
+#pragma unroll
+          for (int i = 0; i < 8; i++) x = __builtin_fmaf(q[i], f[i], x);
+          x += dpp_f<0xB1>(x);
+          x += dpp_f<0x4E>(x);
+          x += dpp_f<0x141>(x);
+          if constexpr (L == 16) x += dpp_f<0x140>(x);
+          sc[i0 + u] = sub + 64 / L * (i0 + u) < here ? x * scale[u] : -__builtin_inff();
+          top = __builtin_fmaxf(top, sc[i0 + u]);
+        }
+      }
+#pragma unroll
+      for (int x = L; x < 64; x <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, x));
+      const float ref = top == -__builtin_inff() ? 0.0f : top;
+      const float alpha = __builtin_amdgcn_exp2f(m - ref);  // 0 for the first scores
+      m = top;
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < 8; i++) o[i] *= alpha;
+#pragma unroll
+      for (int i0 = 0; i0 < N; i0 += kAhead) {
+        int my = sub;
+        if constexpr (kAhead < N) asm volatile("" : "+v"(my)::"memory");  // (no more loads and places ahead than there are registers)
+        v4i_r w[kAhead];
+        float scale[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+          const int key = min(my + 64 / L * (i0 + u), here - 1);
+          w[u] = fetch(vr, key * vj);
+          scale[u] = coded ? s.vs[hk * s.vsh + (key0 + key) * s.vsj] : 1.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+          const float p = __builtin_amdgcn_exp2f(sc[i0 + u] - ref), weight = p * scale[u];
+          float f[8];
+          widen(w[u], f);
+          l += p;
+          const bool seen = sub + 64 / L * (i0 + u) < here;
+#pragma unroll
+          for (int i = 0; i < 8; i++) o[i] = seen ? __builtin_fmaf(weight, f[i], o[i]) : o[i];
+        }
+      }
+    }
+  };
+#pragma unroll 1
+  for (int t = src0; t < src0 + nsrc; t++) {
+    if constexpr (CODES) {
+      if (a.src[t].ks) {
+        walk(a.src[t], std::true_type());
+        continue;
+      }
+    }
+    walk(a.src[t], std::false_type());
+  }
+#pragma unroll
+  for (int x = L; x < 64; x <<= 1) {
+    l += __shfl_xor(l, x);
+#pragma unroll
+    for (int i = 0; i < 8; i++) o[i] += __shfl_xor(o[i], x);
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  if (lane < L)
+    *reinterpret_cast<out8*>(a.o + b * a.sob + h * a.soh + qi * a.soi + 8 * chunk) =
+        out8{pack2<DT>(o[0] * inv, o[1] * inv), pack2<DT>(o[2] * inv, o[3] * inv), pack2<DT>(o[4] * inv, o[5] * inv),
+             pack2<DT>(o[6] * inv, o[7] * inv)};
+}
+
+// The rows of the lanes whose bits are set, one after another.
+template <int DT, int D, int A, bool CODES>
+__device__ __forceinline__ void mend_rows(int src0, int nsrc, uint64_t lanes, int b, int qi, int h, int lane) {
+  while (lanes != 0) {
+    const int from = __builtin_ctzll(lanes);
+    lanes &= lanes - 1;
+    mend_row<DT, D, A, CODES>(src0, nsrc, __builtin_amdgcn_readlane(b, from), __builtin_amdgcn_readlane(qi, from), __builtin_amdgcn_readlane(h, from), lane);
+  }
+}
+
+// The rows, of L lanes each, in which a lane is `bad`.
+template <int DT, int D, int A, bool CODES, int L>
+__device__ __forceinline__ void mend_lanes(int src0, int nsrc, bool bad, int b, int qi, int h, int lane) {
+  uint64_t lanes = __builtin_amdgcn_ballot_w64(bad);
+  if (__builtin_expect(lanes == 0, 1)) return;
+  uint64_t rows = 0;
+#pragma unroll
+  for (int r = 0; r < 64; r += L) rows |= (lanes >> r & low_bits(L)) != 0 ? 1ull << r : 0;
+  wait_loads();  // (these rows' results are written before they are written again)
+  mend_rows<DT, D, A, CODES>(src0, nsrc, rows, b, qi, h, lane);
+}
+
+__device__ __forceinline__ bool finite4(float4 v) {  // (products with zero: 0 or NaN)
+  return __builtin_fmaf(v.x, 0.0f, v.y * 0.0f) + __builtin_fmaf(v.z, 0.0f, v.w * 0.0f) == 0.0f;
+}
+
 // ---------------------------------------------------------------------------------------------
 // Many rows: 128 a workgroup, tiles of 64 keys that its waves share.
 template <int D>
@@ -503,8 +665,9 @@ struct Tile {
 
 // Leaves or writes the results of 32 rows a group of waves holds: wave `w` those of row group w % RW, over part w / RW of the
 // keys.  Each wave scales its output to the common maximum of its row group in LDS (over the tiles, which every wave is done
-// with); the workgroup adds the parts.  `row0`: the workgroup's first row of the unit.
-template <int DT, int D, int RW, typename Core>
+// with); the workgroup adds the parts.  `row0`: the workgroup's first row of the unit.  MEND: the results are final and under a
+// causal limit that hides keys from some of the rows.
+template <int DT, int D, int RW, bool MEND, typename Core>
 __device__ __forceinline__ void join_parts(const RowArgs& a, const RowJob& job, const Core& core, int unit, int split, int row0,
                                            char* smem, float2* stats) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -528,7 +691,9 @@ __device__ __forceinline__ void join_parts(const RowArgs& a, const RowJob& job, 
     }
   lds_barrier();
   const int rows = min(32 * RW, job.rows - row0);
-  for (int item = tid; item < rows * (D / 4); item += kWaves * 64) {
+  for (int item0 = wave * 64; item0 < rows * (D / 4); item0 += kWaves * 64) {  // (the whole wave stays for rows to mend)
+    const bool in = item0 + lane < rows * (D / 4);
+    const int item = in ? item0 + lane : item0;
     const int row = item / (D / 4), c = item % (D / 4), r32 = row % 32, g = row / 32;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float l = 0.0f, mt = -__builtin_inff();
@@ -545,20 +710,23 @@ __device__ __forceinline__ void join_parts(const RowArgs& a, const RowJob& job, 
     int qi, h;
     locate(a, job, unit, row0 + row, b, qi, h);
     if (a.slots) {
+      if (!in) continue;
       const int64_t id = (int64_t)(job.slot0 + split) * a.ids + (b * a.Lq + qi) * a.Hq + h;
       *reinterpret_cast<float4*>(a.po + id * D + 4 * c) = o;
       if (c == 0) a.pml[id] = make_float2(mt, l);
     } else {
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key seen: zeros
-      *reinterpret_cast<uint2*>(a.o + b * a.sob + h * a.soh + qi * a.soi + 4 * c) =
-          make_uint2(pack2<DT>(o.x * inv, o.y * inv), pack2<DT>(o.z * inv, o.w * inv));
+      if (in)
+        *reinterpret_cast<uint2*>(a.o + b * a.sob + h * a.soh + qi * a.soi + 4 * c) =
+            make_uint2(pack2<DT>(o.x * inv, o.y * inv), pack2<DT>(o.z * inv, o.w * inv));
+      if constexpr (MEND) mend_lanes<DT, D, 16, false, D / 4>(job.src0, job.nsrc, in && qi < a.Lq - 1 && !finite4(o) && l == l, (int)b, qi, h, lane);
     }
   }
 }
 
 // One workgroup's rows and tiles.  I8: the job's one source holds int8 codes.  RW: row groups of 32; with 2, two waves share
 // a group and take a tile's first and second 32 keys.
-template <int DT, int D, bool I8, int RW>
+template <int DT, int D, bool I8, int RW, bool MEND>
 __device__ __forceinline__ void attend_rows(const RowArgs& a, const RowJob& job, const KeySource* src, int nsrc, int index, char* smem, float2* stats, float* scale_lds) {
   using T = Tile<D>;
   using R = Rows<D>;
@@ -756,13 +924,14 @@ __device__ __forceinline__ void attend_rows(const RowArgs& a, const RowJob& job,
 
   if constexpr (RW == 2) {
     lds_barrier();  // every wave is done with the tiles
-    join_parts<DT, D, RW>(a, job, core, unit, split, row0, smem, stats);
+    join_parts<DT, D, RW, MEND>(a, job, core, unit, split, row0, smem, stats);
   } else {
     if (!live) return;
     const float ltot = core.total();
     const int h2 = lane >> 5;
-    if (r0 + (lane & 31) >= job.rows) return;
+    const bool in = r0 + (lane & 31) < job.rows;
     if (a.slots) {
+      if (!in) return;
       const int64_t id = (int64_t)(job.slot0 + split) * a.ids + (at.b * a.Lq + at.qi) * a.Hq + at.h;
       float* po = a.po + id * D + 4 * h2;
 #pragma unroll
@@ -775,6 +944,7 @@ __device__ __forceinline__ void attend_rows(const RowArgs& a, const RowJob& job,
       return;
     }
     const float inv = ltot == 0.0f ? 0.0f : 1.0f / ltot;  // no key seen: zeros
+    const bool bad = MEND && in && at.qi < a.Lq - 1 && !core.finite() && ltot == ltot;  // (a NaN among a row's own scores stays)
     // (the two halves of a row trade four values, so that each lane stores eight at once)
     uint16_t* op = a.o + at.b * a.sob + at.h * a.soh + at.qi * a.soi + 8 * h2;
 #pragma unroll
@@ -786,8 +956,15 @@ __device__ __forceinline__ void attend_rows(const RowArgs& a, const RowJob& job,
         for (int i = 0; i < 4; i++) w[i] = pack2<DT>(core.oacc[db][4 * rr + 2 * i] * inv, core.oacc[db][4 * rr + 2 * i + 1] * inv);
         const auto x = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
         const auto y = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
-        *reinterpret_cast<out8*>(op + 32 * db + 8 * rr) = out8{x[0], y[0], x[1], y[1]};
+        if (in) *reinterpret_cast<out8*>(op + 32 * db + 8 * rr) = out8{x[0], y[0], x[1], y[1]};
       }
+    if constexpr (MEND) {
+      const uint64_t lanes = __builtin_amdgcn_ballot_w64(bad);
+      if (__builtin_expect(lanes != 0, 0)) {
+        wait_loads();  // (these rows' results are written before they are written again)
+        mend_rows<DT, D, 16, false>(job.src0, job.nsrc, (lanes | lanes >> 32) & low_bits(32), (int)at.b, at.qi, at.h, lane);
+      }
+    }
   }
 }
 
@@ -805,7 +982,7 @@ struct FewTile {
   static constexpr bool kQL = D == 128;                 // the query rows' fragments lie in LDS too
 };
 
-template <int DT, int D, bool I8>
+template <int DT, int D, bool I8, bool MEND>
 __device__ __forceinline__ void attend_few(const RowArgs& a, const RowJob& job, const KeySource* src, int nsrc, int index, char* smem, char* q_lds, float2* stats, float* scale_lds) {
   using T = FewTile<D>;
   using R = Rows<D>;
@@ -954,18 +1131,20 @@ __device__ __forceinline__ void attend_few(const RowArgs& a, const RowJob& job, 
   }
 
   lds_barrier();
-  join_parts<DT, D, 1>(a, job, core, unit, split, 0, smem, stats);
+  join_parts<DT, D, 1, MEND>(a, job, core, unit, split, 0, smem, stats);
 }
 
-template <int DT, int D, bool I8>
+template <int DT, int D, bool I8, bool MEND>
 __device__ __forceinline__ void attend(const RowArgs& a, const RowJob& job, const KeySource* src, int nsrc, int index, char* smem, char* q_lds, float2* stats, float* scales) {
-  if (job.kind == kFew) attend_few<DT, D, I8>(a, job, src, nsrc, index, smem, q_lds, stats, scales);
-  else if (job.kind == kHalf) attend_rows<DT, D, I8, 2>(a, job, src, nsrc, index, smem, stats, scales);
-  else attend_rows<DT, D, I8, 4>(a, job, src, nsrc, index, smem, stats, scales);
+  if (job.kind == kFew) attend_few<DT, D, I8, MEND>(a, job, src, nsrc, index, smem, q_lds, stats, scales);
+  else if (job.kind == kHalf) attend_rows<DT, D, I8, 2, MEND>(a, job, src, nsrc, index, smem, stats, scales);
+  else attend_rows<DT, D, I8, 4, MEND>(a, job, src, nsrc, index, smem, stats, scales);
 }
 
-// All jobs of a call.  I8: the first one's keys are int8 codes.
-template <int DT, int D, bool I8>
+// All jobs of a call.  I8: the first one's keys are int8 codes (then the own keys' job, where there is one, is a second one, and its
+// results are partials).  MEND: the results are final and under a causal limit with several queries (a kernel apart:
+// within one, calls without a limit took 0.2 us more, 64 samples over 32768 shared keys 61.4 in place of 59.2).
+template <int DT, int D, bool I8, bool MEND>
 __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void row_attention_kernel(const RowArgs a) {
   // one array for all of it: with several, the compiler lets every LDS read wait for the direct loads in flight
@@ -979,11 +1158,11 @@ void row_attention_kernel(const RowArgs a) {
   float* const scales = reinterpret_cast<float*>(lds + tiles + q_bytes + stat_bytes);
   const bool second = a.njobs > 1 && (int64_t)blockIdx.x >= a.job[1].wg0;
   if constexpr (I8) {  // (constant places in the arguments: they are read where they lie)
-    if (!second) attend<DT, D, true>(a, a.job[0], &a.src[0], 1, (int)blockIdx.x, smem, q_lds, stats, scales);
-    else attend<DT, D, false>(a, a.job[1], &a.src[1], 1, (int)(blockIdx.x - a.job[1].wg0), smem, q_lds, stats, scales);
+    if (!second) attend<DT, D, true, false>(a, a.job[0], &a.src[0], 1, (int)blockIdx.x, smem, q_lds, stats, scales);
+    else attend<DT, D, false, false>(a, a.job[1], &a.src[1], 1, (int)(blockIdx.x - a.job[1].wg0), smem, q_lds, stats, scales);
   } else {
     const RowJob& job = a.job[second];
-    attend<DT, D, false>(a, job, &a.src[job.src0], job.nsrc, (int)(blockIdx.x - job.wg0), smem, q_lds, stats, scales);
+    attend<DT, D, false, MEND>(a, job, &a.src[job.src0], job.nsrc, (int)(blockIdx.x - job.wg0), smem, q_lds, stats, scales);
   }
 }
 
@@ -991,8 +1170,10 @@ void row_attention_kernel(const RowArgs a) {
 // Joins the partials of a row: out = sum_s w_s O_s / sum_s w_s l_s, w_s = exp2(m_s - max m).  D / 4 lanes take a row, 16 bytes
 // each, GR such groups share its slots; a slot that saw no key (sum 0) is left out, and a row of such slots is zeros.
 // Short (5 to 6 us, its launch 2): four slots' loads go out together, which took 0.5 us off a slot at a time.
-template <int DT, int D, int GR>
-__global__ __launch_bounds__(256) void row_combine_kernel(const RowArgs a) {
+// MEND: under a causal limit with several queries.  Seven waves a SIMD, which costs the mending a few registers in memory: at the
+// five that it takes otherwise, 64 samples of 4 queries over 9000 and 200 keys took 65.0 us, now 62.7, as without it.
+template <int DT, int D, int GR, bool MEND>
+__global__ __launch_bounds__(256, 7) void row_combine_kernel(const RowArgs a) {
   constexpr int L = D / 4, R = 256 / L / GR;
   const int group = threadIdx.x / L, c = threadIdx.x % L;
   const int64_t id = (int64_t)blockIdx.x * R + group / GR;
@@ -1031,15 +1212,21 @@ __global__ __launch_bounds__(256) void row_combine_kernel(const RowArgs a) {
     part_o[threadIdx.x] = o;
     if (c == 0) part_ml[group] = make_float2(top, l);
     __syncthreads();
-    if (group % GR != 0) return;
+    if constexpr (MEND) {  // (a row's other groups in its first one's wave work along: the wave stays whole for a row to mend)
+      if ((group & -(64 / L)) % GR != 0) return;
+    } else {
+      if (group % GR != 0) return;
+    }
+    const int of = group - group % GR;
+    top = -__builtin_inff();
 #pragma unroll
-    for (int k = 1; k < GR; k++) top = __builtin_fmaxf(top, part_ml[group + k].x);
+    for (int k = 0; k < GR; k++) top = __builtin_fmaxf(top, part_ml[of + k].x);
     l = 0.0f;
     o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int k = 0; k < GR; k++) {
-      const float2 ml = part_ml[group + k];
-      const float4 v = part_o[threadIdx.x + k * L];
+      const float2 ml = part_ml[of + k];
+      const float4 v = part_o[(of + k) * L + c];
       if (ml.y == 0.0f) continue;
       const float w = __builtin_amdgcn_exp2f(ml.x - top);
       l = __builtin_fmaf(w, ml.y, l);
@@ -1049,11 +1236,15 @@ __global__ __launch_bounds__(256) void row_combine_kernel(const RowArgs a) {
       o.w = __builtin_fmaf(w, v.w, o.w);
     }
   }
-  if (id >= a.ids) return;
+  const bool in = id < a.ids && group % GR == 0;
+  if (!MEND && !in) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const int bi = a.by_hq((int)id), h = (int)id - bi * a.Hq, b = a.by_lq(bi), i = bi - b * (int)a.Lq;
-  *reinterpret_cast<uint2*>(a.o + b * a.sob + i * a.soi + h * a.soh + 4 * c) =
-      make_uint2(pack2<DT>(o.x * inv, o.y * inv), pack2<DT>(o.z * inv, o.w * inv));
+  if (in)
+    *reinterpret_cast<uint2*>(a.o + b * a.sob + i * a.soi + h * a.soh + 4 * c) =
+        make_uint2(pack2<DT>(o.x * inv, o.y * inv), pack2<DT>(o.z * inv, o.w * inv));
+  if constexpr (MEND)
+    mend_lanes<DT, D, 4, true, L>(a.src[0].len > 0 ? 0 : 1, a.src[0].len > 0 ? 2 : 1, in && i < a.Lq - 1 && !finite4(o) && l == l, b, i, h, threadIdx.x & 63);
 }
 
 // How a call runs: its jobs, and how many ranges of tiles each unit's keys are split into.
@@ -1171,8 +1362,14 @@ bool plan_shape(int64_t B, int64_t Hq, int64_t Hkv, int64_t Lq, int64_t Lp, int6
 
 template <int DT, int D>
 int launch_rows(const RowArgs& a, int64_t wgs, bool i8, hipStream_t st) {
-  if (i8) hipLaunchKernelGGL((row_attention_kernel<DT, D, true>), dim3((unsigned)wgs), dim3(kWaves * 64), 0, st, a);
-  else hipLaunchKernelGGL((row_attention_kernel<DT, D, false>), dim3((unsigned)wgs), dim3(kWaves * 64), 0, st, a);
+  const bool mend = a.src[1].causal && a.Lq > 1 && a.src[1].len > 0;  // (a single query sees all of its own keys)
+  auto attention = [&](auto i8_c, auto mend_c) {
+    hipLaunchKernelGGL((row_attention_kernel<DT, D, decltype(i8_c)::value, decltype(mend_c)::value>), dim3((unsigned)wgs),
+                       dim3(kWaves * 64), 0, st, a);
+  };
+  if (i8) attention(std::true_type(), std::false_type());
+  else if (mend && a.slots == 0) attention(std::false_type(), std::true_type());
+  else attention(std::false_type(), std::false_type());
   const int rc = HN_LAUNCH_CHECK("row_attention_kernel");
   if (rc != HN_OK) return rc;
   if (a.slots == 0) return HN_OK;
@@ -1180,7 +1377,9 @@ int launch_rows(const RowArgs& a, int64_t wgs, bool i8, hipStream_t st) {
   constexpr int most = 256 / (D / 4);
   auto combine = [&](auto gr_c) {
     constexpr int GR = decltype(gr_c)::value, R = most / GR;
-    hipLaunchKernelGGL((row_combine_kernel<DT, D, GR>), dim3((unsigned)((a.ids + R - 1) / R)), dim3(256), 0, st, a);
+    const dim3 grid((unsigned)((a.ids + R - 1) / R)), block(256);
+    if (mend) hipLaunchKernelGGL((row_combine_kernel<DT, D, GR, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((row_combine_kernel<DT, D, GR, false>), grid, block, 0, st, a);
   };
   if (a.slots >= 16) combine(std::integral_constant<int, 8>());
   else if (a.slots >= 4) combine(std::integral_constant<int, 4>());

@@ -444,8 +444,9 @@ def prefix_attention(q, prefix, k, v, own_lengths=None, *, causal=False, scale=N
     type that `kv.dequantize_kv` makes.
     `own_lengths` (int32 or int64 [B], on the device): sample b's own keys are its first own_lengths[b] of Ls (clamped to
     0..Ls; None: all).  `causal`: a sample's last Lq own keys are its queries' own, and query i sees its own keys up to
-    own_lengths[b] - Lq + i (none where that is negative); the keys that only later queries see must be finite.  A query that
-    sees no key at all gives zeros.  bf16 or fp16, head dim 64 or 128, any strides; `scale` defaults to D ** -0.5."""
+    own_lengths[b] - Lq + i (none where that is negative); keys that it does not see take no part whatever they hold (where later
+    tokens' values are not finite, the rows of nearby queries are worked out a second time).  A query that sees no key at all
+    gives zeros.  bf16 or fp16, head dim 64 or 128, any strides; `scale` defaults to D ** -0.5."""
     qs, ks, out, qo, ko, vo, oo, n = _serving_operands("prefix_attention", q, k, v, own_lengths, out)
     b, lq, hq, d = qs
     ls, hkv = ks[1], ks[2]

@@ -248,8 +248,8 @@ int hn_cross_attention(const void* q, int64_t sqb, int64_t sqh, int64_t sqi, con
  *   or NULL; the same for v.  Without scales k and v are of `dtype`, with them int8 codes of the values
  *   code * scale, not rounded to `dtype`.  Lp keys.
  *   k / v [B, Ls, Hkv, D]: each sample's own keys, lengths[b] of them (as in hn_cross_attention).  causal: the sample's
- *   last Lq keys are its queries' own, and query i sees own keys up to lengths[b] - Lq + i; keys within the length that only
- *   later queries see must be finite.
+ *   last Lq keys are its queries' own, and query i sees own keys up to lengths[b] - Lq + i; what later ones hold stays with
+ *   the queries that see them, also where it is not finite (rows next to such values take longer).
  * Other arguments and results are those of hn_cross_attention; int8 rows are 16-byte aligned too.
  */
 int64_t hn_prefix_attention_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Lq, int64_t Lp, int64_t Ls, int64_t D,

@@ -693,3 +693,59 @@ def test_an_output_whose_single_dims_have_odd_strides(dev):
     assert attention.cross_attention(q, k, v, out=out) is out and torch.equal(out, want)
     out = torch.as_strided(torch.zeros(500, device=dev, dtype=bf), (1, 1, 2, 64), (7, 5, 64, 1))
     assert torch.equal(attention.cross_attention(q[:, :1], k, v, out=out), attention.cross_attention(q[:, :1], k, v))
+
+
+# few, half and whole blocks of rows; one pass, two jobs and split keys; no prefix, a short, a long and an int8 one
+LATER = [(2, 5, 0, 40, 2, 1, 128, False), (1, 12, 0, 3000, 4, 4, 64, False), (2, 20, 0, 90, 4, 2, 64, False), (2, 40, 0, 130, 2, 2, 128, False),
+         (1, 150, 0, 200, 2, 1, 128, False), (2, 100, 33, 160, 4, 2, 64, False), (2, 130, 700, 140, 2, 1, 128, False), (4, 6, 900, 50, 4, 2, 128, False),
+         (3, 9, 500, 70, 2, 2, 128, True), (2, 140, 300, 150, 2, 1, 64, True)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("b,lq,lp,ls,hq,hkv,d,int8", LATER)
+def test_what_a_later_token_holds_stays_with_the_rows_that_see_it(dev, b, lq, lp, ls, hq, hkv, d, int8, dtype):
+    """Under `causal`, infinities and NaN in keys and values from token j0 on: earlier queries' rows are those of the formula,
+    later ones carry what they see, and a value's other dims stay as they are."""
+    from hy_nomas import attention
+
+    q, prefix, k, v, g = prefix_case(dev, b, lq, lp, ls, hq, hkv, d, TYPES[dtype], int8, lq + lp + 3)
+    lengths = torch.full((b,), ls, device=dev)
+    lengths[-1] = ls - 3
+    clean = attention.prefix_attention(q, prefix, k, v, lengths, causal=True)
+    check_prefix(clean, q, prefix, k, v, lengths, True)
+    for j0 in sorted({1, lq // 2, lq - 1}):
+        for what, bad in (("values", "nan"), ("values", "inf"), ("keys", "nan"), ("keys", "inf"), ("both", "-inf")):
+            print(f"later b={b} lq={lq} lp={lp} ls={ls} d={d} int8={int8} {dtype} j0={j0} {what} {bad}", flush=True)
+            kb, vb = k.clone(), v.clone()
+            for i in range(b):
+                n = int(lengths[i])
+                if what != "values":
+                    kb[i, n - lq + j0:n] = float(bad)
+                if what != "keys":
+                    vb[i, n - lq + j0:n, :, 5] = float(bad)
+                if what == "both":
+                    vb[i, n - lq + j0:n] = float(bad)
+            got = attention.prefix_attention(q, prefix, kb, vb, lengths, causal=True)
+            check_prefix(got[:, :j0], q[:, :j0], prefix, k, v, lengths - (lq - j0), True)
+            if what == "values":
+                assert not got[:, j0:, :, 5].isfinite().any()
+                rest = got.clone()
+                rest[..., 5] = clean[..., 5]
+                check_prefix(rest, q, prefix, k, v, lengths, True)
+            elif bad == "nan":
+                assert got[:, j0:].isnan().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("b,lq,ls,hq,hkv,d", [(2, 150, 140, 2, 2, 64), (2, 12, 10, 2, 1, 128), (2, 40, 30, 2, 2, 128), (1, 300, 260, 2, 1, 128)])
+def test_queries_before_the_first_own_key_give_zeros_beside_anything(dev, b, lq, ls, hq, hkv, d):
+    """More queries than own keys and no prefix: the first queries see nothing, whatever the keys of the others hold."""
+    from hy_nomas import attention
+
+    q, prefix, k, v, _ = prefix_case(dev, b, lq, 0, ls, hq, hkv, d, torch.bfloat16, False, lq)
+    for what in (k, v):
+        what[:] = float("nan")
+        got = attention.prefix_attention(q, prefix, k, v, causal=True)
+        assert (got[:, :lq - ls] == 0).all() and got[:, lq - ls:].isnan().all()
+        what[:] = 1.0
