@@ -506,10 +506,10 @@ __device__ __forceinline__ void store_codes(char* row, int swz, int c, v4i_r w) 
 
 // One row's attention again, by a whole wave over the keys that the row sees and no others, in fp32: 64 keys a step, D / 8 lanes a
 // key and 8 dims a lane, for K and V alike.  For rows whose result is not finite under a causal limit although their scores are,
-// so that what a later token's values hold stays with the rows that see it; slow beside the tiles, and rare: 4 x 2000 queries over 8192
-and 2000 keys take 1.1 ms, with a NaN in one sample's last value 11, in the first own value of every sample (where the rows are
-walked again for nothing) 55.  A: keys of a lane whose
-// rows are loaded together (in a kernel of many registers all of a step's).  CODES: a source may hold int8 codes.
+// so that what a later token's values hold stays with the rows that see it; slow beside the tiles, and rare: 4 x 2000 queries
+// over 8192 and 2000 keys take 1.1 ms, with a NaN in one sample's last value 11, in the first own value of every sample (where the
+// rows are walked again for nothing) 55.  A: keys of a lane whose rows are loaded together (in a kernel of many registers all
+// of a step's).  CODES: a source may hold int8 codes.
 template <int DT, int D, int A, bool CODES>
 __device__ __forceinline__ void mend_row(int src0, int nsrc, int b, int qi, int h, int lane) {
   const RowArgs& a = *(const RowArgs*)__builtin_amdgcn_kernarg_segment_ptr();  // (as a reference handed on, the arguments are copied)
