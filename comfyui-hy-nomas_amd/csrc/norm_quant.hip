@@ -8,7 +8,8 @@
 //
 // One pass, bound by memory: a row is read once into registers by WPR waves (one, or four for long rows and for calls of few
 // rows), 8 values a lane and chunk, with non-temporal accesses (plain ones were 3 to 7 % slower over rows that no cache holds);
-// 35200 rows of 4096 values with a residual 166 us, 6.1 TB/s of a copy's 6.6.  The codes do not wait for the row's statistics:
+// 35200 rows of 4096 values with a residual 166 us in bf16, 6.1 TB/s of a copy's 6.6; 164 in fp16; 360 in fp32,
+// 5.2 TB/s.  The codes do not wait for the row's statistics:
 // with t = h w the quotient y / s is t / (max |t| / 127), so each group's quotients come from the group alone and only the scale,
 // max |t| rstd / 127, needs rstd.  Groups
 // whose products lie outside [2^-80, 2^100], where t or its reciprocal could leave fp32's normal range (all-zero and
@@ -253,8 +254,8 @@ __global__ __launch_bounds__(kThreads) void rms_norm_quant_kernel(const NormArgs
   const float rstd = rsqrt_refined(sq / (float)a.D + a.eps);
   uint8_t* qr = a.q + row * a.ldq;
   float* sr = a.s + row * a.lds;
-  // chunk i's channels again as y = h rstd w, for groups the factors are not for
-  auto formula = [&](int i, float* y) {
+  // chunk i's channels again, as t = h w and as y = h rstd w, for groups the factors are not for
+  auto formula = [&](int i, float* t, float* y) {
     Eight<DT> e;
     float w[8];
     e.load(a.r ? (const char*)hr : xr, first + kStep * i);
@@ -263,6 +264,7 @@ __global__ __launch_bounds__(kThreads) void rms_norm_quant_kernel(const NormArgs
     uint32_t p = 0;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
+      t[j] = y[j] * w[j];
       y[j] = y[j] * rstd * w[j];
       p = max(p, magnitude(y[j]));
     }
@@ -280,8 +282,8 @@ __global__ __launch_bounds__(kThreads) void rms_norm_quant_kernel(const NormArgs
     top = 0;
 #pragma unroll 1
     for (int c = first, i = 0; c < chunks; c += kStep, i++) {
-      float y[8];
-      top = max(top, formula(i, y));
+      float again[8], y[8];
+      top = max(top, formula(i, again, y));
     }
     top = wave_max_u(top);
     if constexpr (WPR > 1) {
@@ -293,8 +295,8 @@ __global__ __launch_bounds__(kThreads) void rms_norm_quant_kernel(const NormArgs
     const float sc = plain_scale<KIND>(top);
 #pragma unroll 1
     for (int c = first, i = 0; c < chunks; c += kStep, i++) {
-      float y[8];
-      formula(i, y);
+      float again[8], y[8];
+      formula(i, again, y);
       st_nt8(qr + c * 8, plain_codes<KIND>(y, sc, a.rounding));
     }
     if (first == 0) sr[0] = sc;
@@ -325,25 +327,25 @@ __global__ __launch_bounds__(kThreads) void rms_norm_quant_kernel(const NormArgs
       return;
     }
     // Some group of the wave has no factor (pruned channels, say): it alone takes the formula, so that a group's codes never
-    // depend on what lies in another.
-    const float usable = g.ok ? 1.0f : 0.0f;
+    // depend on what lies in another.  (The products are formed again: kept for here, they slowed the path above by 2 to 4 %.)
+#pragma unroll 1
+    for (int c = first, i = 0; c < chunks; c += kStep, i++) {
+      float again[8], y[8];
+      const uint32_t peak_y = row16_max(formula(i, again, y));
+      uint32_t p = 0;
 #pragma unroll
-    for (int i = 0; i < CPL; i++) {
-      const float f = row_bcast(g.rcp, i);
-      const bool fast = row_bcast(usable, i) != 0.0f;  // the same in the group's 16 lanes
-      const int c = first + kStep * i;
-      if (c < chunks) {
-        if (fast) {
-          st_nt8(qr + c * 8, fast_codes<KIND, DT == HN_DTYPE_F16>(t[i], f, __uint_as_float(peak[i]), a.rounding));
-        } else {
-          float y[8];
-          const float sc = plain_scale<KIND>(row16_max(formula(i, y)));
-          st_nt8(qr + c * 8, plain_codes<KIND>(y, sc, a.rounding));
-          if (k == 0) sr[c / 16] = sc;
-        }
+      for (int j = 0; j < 8; j++) p = max(p, magnitude(again[j]));
+      p = row16_max(p);
+      const GroupFactor<KIND> own(p, rstd);
+      if (own.ok) {  // the same in the group's 16 lanes
+        st_nt8(qr + c * 8, fast_codes<KIND, DT == HN_DTYPE_F16>(again, own.rcp, __uint_as_float(p), a.rounding));
+        if (k == 0) sr[c / 16] = own.scale;
+      } else {
+        const float sc = plain_scale<KIND>(peak_y);
+        st_nt8(qr + c * 8, plain_codes<KIND>(y, sc, a.rounding));
+        if (k == 0) sr[c / 16] = sc;
       }
     }
-    if (k < CPL && has && g.ok) sr[at / 16] = g.scale;
   }
 }
 
@@ -368,8 +370,8 @@ int launch_norm(const NormArgs& a, hipStream_t st) {
 
 template <int DT>
 int dispatch_norm(const NormArgs& a, int kind, bool per_token, hipStream_t st) {
-  // A wave a row where rows fill the chip and are short, else four: 35200 rows of 1024 values 42.7 against 54.0 us, of 4096
-  // 176 against 169, 26400 of 2048 the same.
+  // A wave a row where rows fill the chip and are short, else four: 35200 rows of 1024 values 42.6 against 50.2 us, of 4096
+  // 173.7 against 164.3, 26400 of 2048 64.0 against 62.4, 1500 of 2048 5.9 against 4.7.
   const bool one = a.D <= 2048 && a.M >= 8 * cu_count();
 #define HN_NORM_WPR(K, PT) return one ? launch_norm<DT, K, PT, 1>(a, st) : launch_norm<DT, K, PT, 4>(a, st)
   if (kind == HN_KIND_FP8) {
