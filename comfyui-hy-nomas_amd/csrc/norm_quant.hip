@@ -143,15 +143,33 @@ __device__ __forceinline__ uint2 plain_codes(const float* y, float scale, int ro
                                           : encode8<KIND, HN_ROUND_HALF_AWAY, false>(y, scale);
 }
 
+// The codes of z = t top / peak rounded once: int8 by `rounding`, e4m3 to even.
+template <int KIND, bool STICKY>
+__device__ __forceinline__ uint2 quotient_codes(const float* z, int rounding) {
+  if constexpr (KIND == HN_KIND_FP8) {
+    return make_uint2(e4m3_pack4_hw(z[0], z[1], z[2], z[3]), e4m3_pack4_hw(z[4], z[5], z[6], z[7]));
+  } else {
+    int c[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++)  // STICKY: half away by the float below 0.5, whose sum with a value under a half stays under
+      c[j] = rounding == HN_ROUND_HALF_EVEN ? rne_code_bits(z[j])
+             : STICKY                       ? (int)(z[j] + __builtin_copysignf(0x1.fffffep-2f, z[j]))
+                                            : round_half_away_i8_inrange(z[j]);
+    return make_uint2(pack4_i8(c[0], c[1], c[2], c[3]), pack4_i8(c[4], c[5], c[6], c[7]));
+  }
+}
+
 // t top / peak with the quotient's rounding error mended: where it lies halfway between two codes, as 1 in 2300 does with
 // bf16 values and weights, it is formed exactly and goes to the code that the rounding says.  (A product with top / peak alone
 // gave half of those to the other neighbour.)  A bf16 product h w has 16 bits, so t top is exact, and quotients that are no
 // ties lie further from one than fp32's rounding reaches.
 //
-// WIDE, fp16 values: t has up to 22 bits and t top up to 29, so its low part goes into the remainder, and a quotient may lie
-// within fp32's rounding of a tie.  The last remainder e tells on which side; z is made the odd neighbour of the quotient (the
-// quotient itself where e is 0), which no boundary of codes is, so that the rounding to a code sees what a quotient of
-// unlimited precision would show it.  The half-away sum takes the float below 0.5, whose sum with a value under a half stays under.
+// WIDE, fp16 values: t has up to 22 bits and t top up to 29, so a quotient may lie within fp32's rounding of a tie.  z is within
+// 2^-23 of the quotient, relatively; a lane with a z within four steps of a tie (for e4m3 also one of its subnormals) forms
+// its quotients with the product's low part in the remainder.  The last remainder e then tells on which side the
+// quotient lies, and z becomes its odd neighbour (the quotient itself where e is 0), which no boundary of codes is: the rounding to
+// a code sees what a quotient of unlimited precision would show it.  (35200 rows of 1024 take
+// 42.9 us, 777 of 2560 5.25; 43.9 and 5.75 with every lane doing so, 41.9 and 5.1 with ties left to chance.)
 template <int KIND, bool WIDE>
 __device__ __forceinline__ uint2 fast_codes(const float* t, float rcp, float peak, int rounding) {
   constexpr float top = KIND == HN_KIND_FP8 ? 448.0f : 127.0f;
@@ -159,28 +177,46 @@ __device__ __forceinline__ uint2 fast_codes(const float* t, float rcp, float pea
 #pragma unroll
   for (int j = 0; j < 8; j++) {
     const float n = t[j] * top, q = n * rcp;
-    if constexpr (WIDE) {
-      const float lo = __builtin_fmaf(t[j], top, -n);
-      const float near = __builtin_fmaf(__builtin_fmaf(-q, peak, n) + lo, rcp, q);
-      const float e = __builtin_fmaf(-near, peak, n) + lo;
-      const uint32_t bits = __float_as_uint(near);
-      const uint32_t below = (uint32_t)((int)(bits ^ __float_as_uint(e)) >> 31);  // -1 where the quotient is nearer to zero
-      z[j] = __uint_as_float(e == 0.0f ? bits : (bits + below) | 1u);
-    } else {
-      z[j] = __builtin_fmaf(__builtin_fmaf(-q, peak, n), rcp, q);
-    }
+    z[j] = __builtin_fmaf(__builtin_fmaf(-q, peak, n), rcp, q);
   }
+  if constexpr (!WIDE) return quotient_codes<KIND, false>(z, rounding);
+  uint2 codes;
+  bool near;
   if constexpr (KIND == HN_KIND_FP8) {
-    return make_uint2(e4m3_pack4_hw(z[0], z[1], z[2], z[3]), e4m3_pack4_hw(z[4], z[5], z[6], z[7]));
+    codes = quotient_codes<KIND, false>(z, rounding);
+    uint32_t above = ~0u;
+    float least = 1.0f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {  // a tie: the 20 bits below e4m3's mantissa are 0x80000
+      above = min(above, (__float_as_uint(z[j]) - 0x7fffcu) & 0xfffffu);
+      least = __builtin_fminf(least, __builtin_fabsf(z[j]));
+    }
+    near = above <= 8u || least < 0x1p-6f;
   } else {
+    float off = 0.0f;
     int c[8];
 #pragma unroll
-    for (int j = 0; j < 8; j++)
-      c[j] = rounding == HN_ROUND_HALF_EVEN ? rne_code_bits(z[j])
-             : WIDE                         ? (int)(z[j] + __builtin_copysignf(0x1.fffffep-2f, z[j]))
-                                            : round_half_away_i8_inrange(z[j]);
-    return make_uint2(pack4_i8(c[0], c[1], c[2], c[3]), pack4_i8(c[4], c[5], c[6], c[7]));
+    for (int j = 0; j < 8; j++) {  // away from ties both roundings are the nearest code
+      const float r = __builtin_rintf(z[j]);
+      off = __builtin_fmaxf(off, __builtin_fabsf(z[j] - r));
+      c[j] = (int)r;
+    }
+    codes = make_uint2(pack4_i8(c[0], c[1], c[2], c[3]), pack4_i8(c[4], c[5], c[6], c[7]));
+    near = off >= 0.5f - 0x1p-15f;  // (four steps of a z next to 127)
   }
+  if (__builtin_expect(near, 0)) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const float n = t[j] * top, q = n * rcp, lo = __builtin_fmaf(t[j], top, -n);
+      const float about = __builtin_fmaf(__builtin_fmaf(-q, peak, n) + lo, rcp, q);
+      const float e = __builtin_fmaf(-about, peak, n) + lo;
+      const uint32_t bits = __float_as_uint(about);
+      const uint32_t below = (uint32_t)((int)(bits ^ __float_as_uint(e)) >> 31);  // -1 where the quotient is nearer to zero
+      z[j] = __uint_as_float(e == 0.0f ? bits : (bits + below) | 1u);
+    }
+    codes = quotient_codes<KIND, true>(z, rounding);
+  }
+  return codes;
 }
 
 // WPR waves a row, CPL chunks of 8 values a lane; PT: one scale a row.
