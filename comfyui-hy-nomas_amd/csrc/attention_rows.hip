@@ -6,12 +6,14 @@
 // over the keys j that query (b, i) sees, of K/V head h / (Hq / Hkv); zeros where it sees none.
 //
 // Rows.  The queries that read the same keys are the rows of one matrix: the G = Hq / Hkv heads of a K/V head, all queries of
-// the sample, and for a prefix those of every sample, so that its keys are read once for all.  A workgroup of 4 waves walks
-// keys in tiles with a running maximum and sum: 128 rows, a wave 32, over tiles of 64 keys that the waves share; up to 64 rows,
-// two waves a group of 32 rows and each half a tile's keys; up to 32 rows, every wave all rows and tiles of its own.  With the
-// first kind alone, four calls of up to 64 rows took 17.0, 28.4, 96.9 and 70.8 us (4 samples x 300 keys, 32 heads on 8; 8 samples
-// over 2047 shared and 129 own keys; 64 over 32768 and 600; 16 of 4 queries over 15840 int8 keys and 260, 24 heads), with all
-// three 9.4, 13.3, 64.9 and 45.8.
+// the sample, and for a prefix those of every sample, so that up to 128 rows of all samples share a read of its keys (a short
+// prefix, and one that many own rows walk anyway, is walked for each sample together with its own keys: see plan_rows).  A
+// workgroup of 4 waves walks keys in tiles with a running maximum and sum: 128 rows, a wave 32, over tiles of 64 keys that
+// the waves share; up to 64 rows, two waves a group of 32 rows and each half a tile's keys; up to 32 rows, every wave all rows and
+// tiles of its own.  Each kind in its place in the present kernel, us: four calls (4 samples x 300 keys, 32 heads on 8; 8 samples
+// over 2047 shared and 129 own keys; 64 over 32768 and 600; 16 of 4 queries over 15840 int8 keys and 260, 24 heads) take
+// 10.4, 11.6, 61.3 and 62.5 with the first kind alone, 9.2, 11.9, 61.3 and 48.5 with the third, 9.2, 11.9, 60.9 and 42.7 with all
+// three; 16 x 48 queries over 2000 keys 47.4 in 128-row blocks, 48.7 in half ones, 16 x 24 there 43.2, as few rows 44.3.
 //
 // What bounds it.  Many rows: a wave's chain of products and exponentials, of which two waves a SIMD hide a part; 4 x 2000
 // queries of 32 heads on 8 over 8192 shared keys 1140 us, 1050 TFLOP/s, half the matrix cores' cycles at the clock that the
@@ -26,7 +28,8 @@
 //
 // LDS.  K rows: 16-byte chunk c of row r at c ^ (r & 15) (128 dims) or c ^ ((r >> 1) & 7) (64 dims).  V rows, whose reads take
 // 64 bytes of 4 rows: c ^ (4 (r & 3) + (r & 1)) or c ^ (5 ((r >> 1) & 1)); the low bit spreads the widened int8 rows' writes.
-// Every access spreads over all banks.  Direct-to-LDS loads one tile ahead, two buffers, one barrier a tile; the lane fetches
+// Every read spreads over all banks, and so do the direct loads.  (The widened int8 rows' 16-byte writes do not: 0.24 cycles of
+// conflicts a cycle of LDS access for 16 x 4 queries over 15840 int8 keys, 0.006 without these writes.)  Direct-to-LDS loads one tile ahead, two buffers, one barrier a tile; the lane fetches
 // the logical chunk of its physical slot.
 //
 // int8 keys (a history as stored) pass through registers: loaded a tile ahead, widened once a workgroup, while the score products
@@ -40,7 +43,10 @@
 // finite, and with keys that it does not see, is walked again by a wave over the keys that it sees (`mend_row`).
 //
 // Splits.  Where the rows leave compute units idle, several workgroups take ranges of the tiles and leave fp32 partials with
-// their reference maximum and sum, which row_combine_kernel joins; a prefix and the samples' own keys are joined the same way.
+// their reference maximum and sum, which row_combine_kernel joins; a prefix and the samples' own keys are joined the same way.  An
+// int8 prefix is always a job of its own (a workgroup's tiles are of one type), so each row of such a call leaves at least two
+// partials of D + 2 floats: 2 GB for 16 x 4096 queries of 32 heads, some 0.7 of the 13 ms that they take over 8192 shared and 4096
+// own keys.  Next to a short prefix it shows: 4 x 2000 queries over 64 and 2000 keys 287 us, 178 with a bf16 prefix in one pass.
 //
 // The reference maximum moves only when a tile's maximum exceeds it by more than 8 (base 2), so that the accumulators are
 // rescaled a few times a row; the quotient is the same.
@@ -1258,7 +1264,8 @@ struct RowPlan {
 // of many rows takes a workgroup 1.15 alone on its unit and 2.0 beside another, of half rows 0.85 and 1.4 (int8 keys, which it
 // widens, 0.55 more), a step of few rows 1.4 and 1.9; none is faster than memory brings it (6.2 bytes a ps for the chip).  A
 // round of workgroups adds 3 for its start and end, partials 4.5 and their traffic; the workgroups of a second job fill the
-// places beside the first one's.
+// places beside the first one's.  What these bring from memory is not counted there, as the samples' lengths are not known: with
+// all Ls keys counted, 72 calls whose splits it changes (of some 20000 drawn, 285) took 2 % longer, 6 % with shorter lengths.
 // `merged`: one pass over both sources, which repeats the prefix for every sample, in place of two jobs.
 RowPlan plan_jobs(int64_t B, int64_t Hq, int64_t Hkv, int64_t Lq, int64_t Lp, int64_t Ls, int64_t D, bool i8, bool merged,
                   double* estimate) {

@@ -436,7 +436,8 @@ def _prefix_table(prefix, q, hkv):
 
 def prefix_attention(q, prefix, k, v, own_lengths=None, *, causal=False, scale=None, out=None):
     """Attention of a batch q [B, Lq, Hq, D] over one prefix that all samples share, then each sample's own keys k / v
-    [B or 1, Ls, Hkv, D]; the prefix is read once for all samples.  Query head h reads K/V head h // (Hq // Hkv).  Returns
+    [B or 1, Ls, Hkv, D]; the prefix is held once, and up to 128 rows (heads of a K/V head, queries, samples) share a read of
+    it.  Query head h reads K/V head h // (Hq // Hkv).  Returns
     [B, Lq, Hq, D] (`out` if given, which must not overlap the inputs).
 
     `prefix`: (keys, values), each [Lp, Hkv, D] (or [1, Lp, Hkv, D]) in q's type, or each a pair (int8 codes, fp32 scales

@@ -227,7 +227,7 @@ int hn_segment_attention(const void* q, int64_t sqb, int64_t sqh, int64_t sqi, c
  *   out[b, i, h, :] = sum_j softmax_j(scale * q[b, i, h, :] . k[b, j, h / G, :]) v[b, j, h / G, :],  G = Hq / Hkv,
  * over the keys j of sample b that are seen: j < lengths[b] (device, lengths_bits 32 or 64, clamped to [0, Lk]; NULL: Lk)
  * and mask[b * smb + j] != 0 (device bytes; NULL: all).  Hidden keys and values take no part whatever they hold; a query that
- * sees no key (or scores -inf everywhere) gives zeros.
+ * sees no key (or scores -inf everywhere) gives zeros.  A seen value that is infinite makes its results infinite or NaN.
  * q [B, Lq, Hq, D], k / v [B, Lk, Hkv, D], out [B, Lq, Hq, D] of `dtype` (bf16 or fp16), D 64 or 128 (contiguous), any
  * element strides of batch / head / token (0 repeats a batch) with rows 16-byte aligned (out 8-byte), token strides of
  * k and v in [0, 2^23].  1e-30 < scale < 1e30.  out must not overlap the inputs.  fp32 scores, maxima and sums; probabilities of `dtype` in the
@@ -242,7 +242,7 @@ int hn_cross_attention(const void* q, int64_t sqb, int64_t sqh, int64_t sqi, con
                        float scale, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
- * Attention of a batch over one prefix that all samples share, computed once for all, then each sample's own keys
+ * Attention of a batch over one prefix that all samples share, held once for all, then each sample's own keys
  * (the shared history of hy_nomas/model.py:199-223, with the int8 form of hy_nomas/world.py:83-90 read as it is stored).
  *   prefix [12], a host table: k pointer, its head and token strides; k scales (fp32) and their head and token strides,
  *   or NULL; the same for v.  Without scales k and v are of `dtype`, with them int8 codes of the values
